@@ -108,6 +108,23 @@ __device__ __forceinline__ void lane_sums(u32x4_t* raw, float R, float k, float 
     __builtin_amdgcn_sched_barrier(0);
   }
 }
+// Long sums are added up in two steps: pieces of kPiece vectors a lane, 32 terms at most, and the pieces.  (In one, a
+// lane's rounding grew with the row: 7e-6 in the logarithm at 131072 columns of few values, 1e-3 at 2^24.)
+constexpr int kPiece = 4;
+
+// lane_sums in pieces
+template <typename T, int V0, int V1, bool ENT, bool FMA>
+__device__ __forceinline__ void lane_pieces(u32x4_t* raw, float R, float k, float c, float& s, float& t) {
+  if constexpr (V0 < V1) {
+    constexpr int E = V0 + kPiece < V1 ? V0 + kPiece : V1;
+    float ps = 0.f, pt = 0.f;
+    lane_sums<T, V0, E, ENT, FMA>(raw, R, k, c, ps, pt);
+    s += ps;
+    if (ENT) t += pt;
+    lane_pieces<T, E, V1, ENT, FMA>(raw, R, k, c, s, t);
+  }
+}
+
 // (m, s, t) of a piece added to S, Tt against the finite reference M.  In two halves: s may be as large as the factor
 // is small (values of a hundred behind a masked front, summed against 0, beside a reference of their own size).
 __device__ __forceinline__ void join_piece(float m, float s, float t, float M, float c, float& S, float& Tt) {
@@ -196,9 +213,9 @@ __device__ __forceinline__ void part_stats(u32x4_t* raw, int tid, int len, float
   R = wave_reference<T>(raw, c, s);
   t = 0.f;
   const float k = rintf(R * c);
-  lane_sums<T, 0, Q, ENT, true>(raw, 0.f, k, c, s, t);
+  lane_pieces<T, 0, Q, ENT, true>(raw, 0.f, k, c, s, t);
   if (Q) fix_part<T, TPB, NV, Q>(raw, tid, 0, len);
-  lane_sums<T, Q, NV, ENT, true>(raw, 0.f, k, c, s, t);
+  lane_pieces<T, Q, NV, ENT, true>(raw, 0.f, k, c, s, t);
   const float off = __builtin_fmaf(-R, c, k), f = exp2_fast(off);
   if (ENT) t = f * __builtin_fmaf(s, off, t);
   s *= f;
@@ -208,7 +225,7 @@ __device__ __forceinline__ void part_stats(u32x4_t* raw, int tid, int len, float
   if (TPB > 64) __syncthreads();
   R = block_max<TPB>(lane_max<T, NV>(raw), red);
   s = t = 0.f;
-  lane_sums<T, 0, NV, ENT, false>(raw, R, 0.f, c, s, t);
+  lane_pieces<T, 0, NV, ENT, false>(raw, R, 0.f, c, s, t);
   join_waves<TPB, ENT>(c, red, R, s, t);
 }
 
@@ -471,7 +488,7 @@ __global__ void __launch_bounds__(64) vocab_stats_kernel(const VocabArgs a) {
 // value (the K-th largest of the lanes' own maxima so far), and where it reaches that, the vector's number is noted.
 // The threshold is formed behind the first piece and again behind the 4th, 16th and last, so a few times K vectors are
 // noted; these are read again and their values that reach the last threshold are ranked.
-constexpr int kChunk = 4;
+constexpr int kChunk = kPiece;
 constexpr int kNoted = 4096;   // vectors noted: all that fewer than K lanes can hold, 64 each
 constexpr int kCands = 512;    // values ranked
 constexpr int kTopVecs = 64;   // vectors of a thread in a part with top alternatives
@@ -635,17 +652,22 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
     float x_tok = 0.f;
     if (a.nparts == 1 && threadIdx.x == 0) x_tok = token_logit<T>(a, row, tok);
     if (TOP && threadIdx.x == 0) top.n_noted = top.n_cands = 0;  // the first use is behind block_kth's barriers
-    // as part_stats: a reference from the wave's first vector, sums of 2^(x c - k)
+    // as part_stats: a reference from the wave's first vector, sums of 2^(x c - k); those of the pieces are added up in
+    // 64 bits (a lane of a row of 2^24 columns adds 2048 of them and more)
     float s, R = wave_reference<T>(raw, a.c, s), t = 0.f, logs;
     const float k = rintf(R * a.c);
+    double sum = s, weighted = 0.;
     float lmax = -INFINITY, thr = -INFINITY;
     for (int piece = 0, at = p0; at < end; at += STEP, ++piece) {
       if (at + STEP < end) load_piece<T>(x, tid, at + STEP, end, next);
       if (at + STEP > end) fix_part<T, 256, kChunk, 0>(raw, tid, at, end);
       float vm[kChunk];
       vm[2] = vm[3] = -INFINITY;
-      lane_sums<T, 0, 2, ENT, true, TOP>(raw, 0.f, k, a.c, s, t, vm);
-      if (at + STEP / 2 < end) lane_sums<T, 2, 4, ENT, true, TOP>(raw, 0.f, k, a.c, s, t, vm);  // uniform
+      float ps = 0.f, pt = 0.f;
+      lane_sums<T, 0, 2, ENT, true, TOP>(raw, 0.f, k, a.c, ps, pt, vm);
+      if (at + STEP / 2 < end) lane_sums<T, 2, 4, ENT, true, TOP>(raw, 0.f, k, a.c, ps, pt, vm);  // uniform
+      sum += ps;
+      if (ENT) weighted += pt;
       if (TOP) {
 #pragma unroll
         for (int v = 0; v < kChunk; ++v) lmax = fmaxf(lmax, vm[v]);
@@ -661,6 +683,8 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
 #pragma unroll
       for (int v = 0; v < kChunk; ++v) raw[v] = next[v];
     }
+    s = (float)sum;
+    t = (float)weighted;
     const float off = __builtin_fmaf(-R, a.c, k), f = exp2_fast(off);
     if (ENT) t = f * __builtin_fmaf(s, off, t);
     s *= f;
@@ -674,12 +698,17 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
         m = fmaxf(m, lane_max<T, kChunk>(raw));
       }
       R = block_max<256>(m, red);
-      s = t = 0.f;
+      sum = weighted = 0.;
       for (int at = p0; at < end; at += STEP) {
         load_part<T, 256, kChunk, 0>(x, tid, at, end, raw);
         fix_part<T, 256, kChunk, 0>(raw, tid, at, end);
-        lane_sums<T, 0, kChunk, ENT, false>(raw, R, 0.f, a.c, s, t);
+        float ps = 0.f, pt = 0.f;
+        lane_sums<T, 0, kChunk, ENT, false>(raw, R, 0.f, a.c, ps, pt);
+        sum += ps;
+        if (ENT) weighted += pt;
       }
+      s = (float)sum;
+      t = (float)weighted;
       join_waves<256, ENT>(a.c, red, R, s, t);
     }
     if (threadIdx.x == 0) {
