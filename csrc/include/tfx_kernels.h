@@ -445,7 +445,7 @@ struct VocabArgs {
   float scale = 1.f, c = 1.f;     // 1 / T, log2(e) / T
   float* logp = nullptr;          // [rows] (null: not wanted)
   float* ent = nullptr;           // [rows] (null: not wanted)
-  float* stats = nullptr;         // [rows][4]: max, 1 / sum, log sum, entropy (null: not wanted)
+  float* stats = nullptr;         // [rows][4]: a reference near the maximum, 1 / sum, log sum, entropy (null: not wanted)
   float* top_logp = nullptr;      // [rows][K]
   int64_t* top_ids = nullptr;     // [rows][K]
   int K = 0;                      // at most kVocabMaxTop

@@ -66,32 +66,39 @@ __device__ __forceinline__ void fix_part(u32x4_t* raw, int t, int p0, int end) {
   }
 }
 
-template <typename T, int NV>
+// ASIDE: in a branch, here and below
+template <typename T, int NV, bool ASIDE = false>
 __device__ __forceinline__ float lane_max(u32x4_t* raw) {
   constexpr int N = Vec<T>::N;
   float m = -INFINITY;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     float f[N];
-    vec_unpack_again<T>(raw[v], f);
+    if (ASIDE) vec_unpack_aside<T>(raw[v], f);
+    else vec_unpack_again<T>(raw[v], f);
 #pragma unroll
     for (int j = 0; j < N; j += 2) m = fmaxf(m, fmaxf(f[j], f[j + 1]));
+    if (ASIDE) __builtin_amdgcn_sched_barrier(0);
   }
   return m;
 }
+
+// v is formed here: where only one side of a branch needs it the compiler would form it there, out of every term
+__device__ __forceinline__ void form_here(float& v) { asm volatile("" : "+v"(v)); }
 
 // s += sum 2^d, t += sum 2^d d over the lane's elements, d = (x - R) c.
 // FMA: d + (R c - k) = x c - k in one rounding, with k the whole number next to R c; the caller takes the
 // fraction out again.
 // MAX: vm[v] = the largest of vector v.
-template <typename T, int V0, int V1, bool ENT, bool FMA, bool MAX = false>
+template <typename T, int V0, int V1, bool ENT, bool FMA, bool MAX = false, bool ASIDE = false>
 __device__ __forceinline__ void lane_sums(u32x4_t* raw, float R, float k, float c, float& s, float& t,
                                           float* vm = nullptr) {
   constexpr int N = Vec<T>::N;
 #pragma unroll
   for (int v = V0; v < V1; ++v) {
     float f[N];
-    vec_unpack_again<T>(raw[v], f);
+    if (ASIDE) vec_unpack_aside<T>(raw[v], f);
+    else vec_unpack_again<T>(raw[v], f);
     if (MAX) {
       vm[v] = f[0];
 #pragma unroll
@@ -105,34 +112,17 @@ __device__ __forceinline__ void lane_sums(u32x4_t* raw, float R, float k, float 
       if (ENT) t = __builtin_fmaf(e, fmaxf(d, kLow), t);
     }
     // one vector's unpacked values at a time: spread over all vectors they cost twice the registers
+    form_here(s);
+    if (ENT) form_here(t);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-// Long sums are added up in two steps: pieces of kPiece vectors a lane, 32 terms at most, and the pieces.  (In one, a
-// lane's rounding grew with the row: 7e-6 in the logarithm at 131072 columns of few values, 1e-3 at 2^24.)
-constexpr int kPiece = 4;
-
-// lane_sums in pieces
-template <typename T, int V0, int V1, bool ENT, bool FMA>
-__device__ __forceinline__ void lane_pieces(u32x4_t* raw, float R, float k, float c, float& s, float& t) {
-  if constexpr (V0 < V1) {
-    constexpr int E = V0 + kPiece < V1 ? V0 + kPiece : V1;
-    float ps = 0.f, pt = 0.f;
-    lane_sums<T, V0, E, ENT, FMA>(raw, R, k, c, ps, pt);
-    s += ps;
-    if (ENT) t += pt;
-    lane_pieces<T, E, V1, ENT, FMA>(raw, R, k, c, s, t);
-  }
-}
-
-// (m, s, t) of a piece added to S, Tt against the finite reference M.  In two halves: s may be as large as the factor
-// is small (values of a hundred behind a masked front, summed against 0, beside a reference of their own size).
+// (m, s, t) of a piece added to S, Tt against the finite reference M, at least m
 __device__ __forceinline__ void join_piece(float m, float s, float t, float M, float c, float& S, float& Tt) {
   const float d = fmaxf((m - M) * c, kLow);
-  const float h = s == 0.f ? 0.f : exp2_fast(0.5f * d);
-  const float hs = s == 0.f ? 0.f : s * h;
-  S += hs * h;
-  Tt += s == 0.f ? 0.f : h * __builtin_fmaf(hs, d, h * t);
+  const float h = s == 0.f ? 0.f : exp2_fast(d);
+  S += s == 0.f ? 0.f : s * h;
+  Tt += s == 0.f ? 0.f : h * __builtin_fmaf(s, d, t);
 }
 
 // the waves' (R, s, t) joined, in every thread; red: 3 * TPB / 64 floats
@@ -142,8 +132,6 @@ __device__ __forceinline__ void join_waves(float c, float* red, float& R, float&
   s = wave64_sum(s);
   if (ENT) t = wave64_sum(t);
   if (W == 1) return;
-  // a reference far below (d of 40 and more, whose rounding alone is some 1e-6 of 2^d): NaN, and no sum is in range
-  s = s <= 1e12f ? s : NAN;
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) red[w] = R, red[W + w] = s, red[2 * W + w] = t;
   __syncthreads();
@@ -173,35 +161,44 @@ __device__ __forceinline__ float block_max(float m, float* red) {
   return finite_max(m);
 }
 
-// Of n values: a sum (and weighted sum) that lost nothing to f32's range against its reference (of NaN: false), and
-// whose reference is near: where one value makes up the sum, its distance d from the reference goes into both log s and
-// t / s, and what their roundings leave of it stays in the entropy (d of up to ln 4 n: 8 nats for 600 values, 13 for
-// 131072; within 2e-5 at that).
-__device__ __forceinline__ bool sum_in_range(float s, float t, int n) {
-  return s >= 0.0625f && s <= 4.f * (float)n && fabsf(t) <= 1e30f;
+// Long sums are added up in two steps: pieces of kPiece vectors a lane, 32 terms at most, and the pieces.  (In one, a
+// lane's rounding grew with the row: 7e-6 in the logarithm at 131072 columns of few values, 1e-3 at 2^24.)
+constexpr int kPiece = 4;
+
+// No maximum is looked for first: a wave sums against a reference R, the largest value of its first vector, which is
+// there first.  Whether R was near enough shows in the pieces' sums: one of up to n terms of about 2^0 and less is at
+// most sqrt(2) n against 2^k, k the whole number next to R c, and one above 1.5 n holds a value above R.  Then the wave
+// takes a new reference from what it holds.  So no value is more than 2^5.6 beside its wave's reference, 3.9 nats: what
+// the f32 roundings of log s and t / s leave of that distance in log p and the entropy is some 1e-6 at most.
+template <typename T>
+constexpr float kPieceMost = 1.5f * kPiece * Vec<T>::N;
+
+// may be a reference: rintf(m c) is exact (of -inf: no)
+__device__ __forceinline__ bool near_zero(float m, float c) { return fabsf(m * c) <= 16777216.f; }
+
+__device__ __forceinline__ float wave_uniform(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
 }
 
-// The reference of a wave's sums, the largest value of its first vector, and what its sum starts at.
-// Where the vector holds nothing (all -inf), or values so far out that rintf(R c) would not be exact, the reference is
-// 0 and the sum starts at kThere: whatever of the wave's values is lost beside 2^0, the joined sum is then one against
-// 0 or more, and leaves the range below where they would count (logits about -200 behind a masked front).  In range
-// kThere is less than 1e-18 of the sum.
-constexpr float kThere = 1e-24f;
-template <typename T>
-__device__ __forceinline__ float wave_reference(u32x4_t* raw, float c, float& s) {
-  const float m = wave64_max(lane_max<T, 1>(raw));
-  const bool near = fabsf(m * c) <= 16777216.f;  // of -inf: false
-  s = near ? 0.f : kThere;
-  return near ? m : 0.f;
+// lane_sums in pieces; big: at least the largest piece's sum
+template <typename T, int V0, int V1, bool ENT, bool FMA>
+__device__ __forceinline__ void lane_pieces(u32x4_t* raw, float R, float k, float c, float& s, float& t, float& big) {
+  if constexpr (V0 < V1) {
+    constexpr int E = V0 + kPiece < V1 ? V0 + kPiece : V1;
+    float ps = 0.f, pt = 0.f;
+    lane_sums<T, V0, E, ENT, FMA, false, !FMA>(raw, R, k, c, ps, pt);
+    s += ps;
+    if (ENT) t += pt;
+    big = fmaxf(big, ps);
+    lane_pieces<T, E, V1, ENT, FMA>(raw, R, k, c, s, t, big);
+  }
 }
 
 // A reference R, sum and weighted sum of the block's part, in every thread: s = sum 2^d, t = sum 2^d d with
 // d = (x - R) c.
 //
-// R need not be the maximum, only near enough for f32's range: each wave takes the largest value of its first
-// vector, which is there first, and sums in one pass over the rest with no maximum to find, against 2^k with k the
-// whole number next to R c (joined without loss).  Where that was not near enough or the row holds NaN or nothing, the
-// block goes over its registers again against the maximum.
+// One pass in FMA form; a wave whose reference was too low, or whose first vector had none (all masked, NaN, or far
+// out), goes over its registers again, against their maximum.  NaN and +inf make s NaN.
 // Instructions an element in bf16: unpack, fma, exp2 (4 slots), add; against the maximum two more for that and
 // one for the difference.
 // The part comes as load_part left it and is whole afterwards.
@@ -210,22 +207,23 @@ __device__ __forceinline__ void part_stats(u32x4_t* raw, int tid, int len, float
                                            float& t) {
   constexpr int Q = sure_vectors(NV);
   if (Q == 0) fix_part<T, TPB, NV, 0>(raw, tid, 0, len);
-  R = wave_reference<T>(raw, c, s);
-  t = 0.f;
-  const float k = rintf(R * c);
-  lane_pieces<T, 0, Q, ENT, true>(raw, 0.f, k, c, s, t);
-  if (Q) fix_part<T, TPB, NV, Q>(raw, tid, 0, len);
-  lane_pieces<T, Q, NV, ENT, true>(raw, 0.f, k, c, s, t);
-  const float off = __builtin_fmaf(-R, c, k), f = exp2_fast(off);
-  if (ENT) t = f * __builtin_fmaf(s, off, t);
-  s *= f;
-  join_waves<TPB, ENT>(c, red, R, s, t);
-  // (for the entropy nearer still: here it costs no second reading)
-  if (sum_in_range(s, t, len) && (!ENT || t <= 8.f * s)) return;
-  if (TPB > 64) __syncthreads();
-  R = block_max<TPB>(lane_max<T, NV>(raw), red);
+  R = wave_uniform(wave64_max(lane_max<T, 1>(raw)));
+  const bool near = near_zero(R, c);
+  const float k = near ? rintf(R * c) : 0.f;
+  float big = near ? 0.f : INFINITY;
   s = t = 0.f;
-  lane_pieces<T, 0, NV, ENT, false>(raw, R, 0.f, c, s, t);
+  lane_pieces<T, 0, Q, ENT, true>(raw, 0.f, k, c, s, t, big);
+  if (Q) fix_part<T, TPB, NV, Q>(raw, tid, 0, len);
+  lane_pieces<T, Q, NV, ENT, true>(raw, 0.f, k, c, s, t, big);
+  if (__ballot(big > kPieceMost<T>)) {
+    R = wave_uniform(finite_max(wave64_max(lane_max<T, NV, true>(raw))));
+    s = t = 0.f;
+    lane_pieces<T, 0, NV, ENT, false>(raw, R, 0.f, c, s, t, big);
+  } else {
+    const float off = __builtin_fmaf(-R, c, k), f = exp2_fast(off);
+    if (ENT) t = f * __builtin_fmaf(s, off, t);
+    s *= f;
+  }
   join_waves<TPB, ENT>(c, red, R, s, t);
 }
 
@@ -394,8 +392,11 @@ __device__ __forceinline__ void put_row(const VocabArgs& a, int row, float x_tok
   const bool empty = s == 0.f;  // every logit -inf
   logs = empty ? INFINITY : logf(s);
   const float inv = empty ? 0.f : 1.f / s;
-  const float H = empty ? 0.f : logs - kLn2 * t * inv;
-  if (a.logp) a.logp[row] = empty ? x_tok : (x_tok - M) * a.scale - logs;
+  // H = log s - ln2 t / s.  Where one value makes up the sum both are its distance from M: a whole number of halvings is
+  // taken off s and t / s alike, in front of the roundings.
+  const float e = rintf(fmaxf(t * inv, 0.f));
+  const float H = empty ? 0.f : e == 0.f ? logs - kLn2 * t * inv : logf(__builtin_ldexpf(s, -(int)e)) + kLn2 * (__builtin_fmaf(e, s, -t) * inv);
+  if (a.logp) a.logp[row] = empty ? x_tok : __builtin_fmaf(x_tok - M, a.scale, -logs);
   if (a.ent) a.ent[row] = H;
   if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(M, inv, empty ? 0.f : logs, H);
 }
@@ -429,7 +430,7 @@ __device__ __forceinline__ float token_logit(const VocabArgs& a, int row, int64_
 
 __device__ __forceinline__ void put_top(const VocabArgs& a, int row, int r, uint64_t key, float M, float logs) {
   const float x = order_val((uint32_t)(key >> 32));
-  a.top_logp[(int64_t)row * a.K + r] = (x - M) * a.scale - logs;
+  a.top_logp[(int64_t)row * a.K + r] = __builtin_fmaf(x - M, a.scale, -logs);
   a.top_ids[(int64_t)row * a.K + r] = (int64_t)(uint32_t)~(uint32_t)key;
 }
 
@@ -631,8 +632,51 @@ __device__ __forceinline__ void load_piece(const T* row, int t, int p0, int end,
   load_part<T, 256, kChunk, 0, true>(row, thread_again(t), p0, end, raw);
 }
 
+// A wave's sums over the pieces so far, lane by lane: s = sum 2^(x c - k), t = sum 2^(x c - k) (x c - k), k the whole
+// number next to R c.  In 64 bits: a lane of a row of 2^24 columns adds 2048 pieces and more.
+struct Running {
+  double s = 0., t = 0.;
+  float R = 0.f, k = 0.f;
+  bool there = false;      // there is a reference
+  float far = -INFINITY;   // the largest value met without one that is too far out to be one itself
+};
+
+// The piece at `at`, whose sums ps, pt are against a reference that is too low, or none: the wave takes the piece's
+// maximum, and what it has so far is brought to that without a rounding.  The piece is read again: kept for this in its
+// registers it cost every piece more than this costs the few (4096 rows of 50000 in bf16, top 5: 93 us, read again 88).
+// vm: its vectors' maxima, if they are known.
+template <typename T, bool ENT>
+__device__ __forceinline__ void refer_again(const T* x, int tid, int at, int end, const float* vm, float c, Running& w,
+                                            float& ps, float& pt) {
+  u32x4_t raw[kChunk];
+  load_part<T, 256, kChunk, 0>(x, thread_again(tid), at, end, raw);
+  fix_part<T, 256, kChunk, 0>(raw, tid, at, end);
+  const float lm = vm ? fmaxf(fmaxf(vm[0], vm[1]), fmaxf(vm[2], vm[3])) : lane_max<T, kChunk>(raw);
+  const float m = wave_uniform(wave64_max(lm));
+  if (!near_zero(m, c)) {  // (of all masked: ps is 0, or NaN; of +inf and far out with a reference: ps is inf or NaN)
+    if (!w.there) w.far = fmaxf(w.far, m);
+    return;
+  }
+  if (w.there && m <= w.R) return;
+  const float k = rintf(m * c);
+  if (w.there) {
+    const double f = ldexp(1., (int)fmaxf(w.k - k, -1000.f));
+    if (ENT) w.t = f * (w.t + w.s * (double)(w.k - k));
+    w.s *= f;
+  } else if ((m - w.far) * c < 160.f) {  // what was far out may count after all
+    w.s = NAN;
+  }
+  w.R = m;
+  w.k = k;
+  w.there = true;
+  ps = pt = 0.f;
+  lane_sums<T, 0, kChunk, ENT, true>(raw, 0.f, k, c, ps, pt);
+}
+
+// (with alternatives five blocks a CU: the compiler would take the registers of one more; 16384 rows of 9000 in bf16,
+// top 20: 127 us, with four 150)
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
+__global__ void __launch_bounds__(256, TOP ? 5 : 1) vocab_stream_kernel(const VocabArgs a) {
   constexpr int N = Vec<T>::N, STEP = 256 * N * kChunk;
   __shared__ float red[12];
   __shared__ uint64_t top_lds[TOP ? sizeof(TopState) / 8 : 1];
@@ -652,11 +696,10 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
     float x_tok = 0.f;
     if (a.nparts == 1 && threadIdx.x == 0) x_tok = token_logit<T>(a, row, tok);
     if (TOP && threadIdx.x == 0) top.n_noted = top.n_cands = 0;  // the first use is behind block_kth's barriers
-    // as part_stats: a reference from the wave's first vector, sums of 2^(x c - k); those of the pieces are added up in
-    // 64 bits (a lane of a row of 2^24 columns adds 2048 of them and more)
-    float s, R = wave_reference<T>(raw, a.c, s), t = 0.f, logs;
-    const float k = rintf(R * a.c);
-    double sum = s, weighted = 0.;
+    // as part_stats: a reference from the wave's first vector, sums of 2^(x c - k)
+    Running w;
+    float s, t = 0.f, logs, R = wave_uniform(wave64_max(lane_max<T, 1>(raw)));
+    if (near_zero(R, a.c)) w.there = true, w.R = R, w.k = rintf(R * a.c);
     float lmax = -INFINITY, thr = -INFINITY;
     for (int piece = 0, at = p0; at < end; at += STEP, ++piece) {
       if (at + STEP < end) load_piece<T>(x, tid, at + STEP, end, next);
@@ -664,10 +707,11 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
       float vm[kChunk];
       vm[2] = vm[3] = -INFINITY;
       float ps = 0.f, pt = 0.f;
-      lane_sums<T, 0, 2, ENT, true, TOP>(raw, 0.f, k, a.c, ps, pt, vm);
-      if (at + STEP / 2 < end) lane_sums<T, 2, 4, ENT, true, TOP>(raw, 0.f, k, a.c, ps, pt, vm);  // uniform
-      sum += ps;
-      if (ENT) weighted += pt;
+      lane_sums<T, 0, 2, ENT, true, TOP>(raw, 0.f, w.k, a.c, ps, pt, vm);
+      if (at + STEP / 2 < end) lane_sums<T, 2, 4, ENT, true, TOP>(raw, 0.f, w.k, a.c, ps, pt, vm);  // uniform
+      if (!w.there || __ballot(!(ps <= kPieceMost<T>))) refer_again<T, ENT>(x, tid, at, end, TOP ? vm : nullptr, a.c, w, ps, pt);
+      w.s += ps;
+      if (ENT) w.t += pt;
       if (TOP) {
 #pragma unroll
         for (int v = 0; v < kChunk; ++v) lmax = fmaxf(lmax, vm[v]);
@@ -683,13 +727,12 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
 #pragma unroll
       for (int v = 0; v < kChunk; ++v) raw[v] = next[v];
     }
-    s = (float)sum;
-    t = (float)weighted;
-    const float off = __builtin_fmaf(-R, a.c, k), f = exp2_fast(off);
-    if (ENT) t = f * __builtin_fmaf(s, off, t);
-    s *= f;
+    const float off = __builtin_fmaf(-w.R, a.c, w.k), f = exp2_fast(off);
+    R = w.R;
+    s = !w.there && w.far > -INFINITY ? NAN : (float)w.s * f;
+    if (ENT) t = f * (float)(w.t + w.s * (double)off);
     join_waves<256, ENT>(a.c, red, R, s, t);
-    if (!sum_in_range(s, t, end - p0)) {  // once more against the maximum, read again
+    if (!(s < INFINITY)) {  // NaN, +inf or values far out: once more against the maximum, read again
       __syncthreads();
       float m = -INFINITY;
       for (int at = p0; at < end; at += STEP) {
@@ -698,17 +741,17 @@ __global__ void __launch_bounds__(256) vocab_stream_kernel(const VocabArgs a) {
         m = fmaxf(m, lane_max<T, kChunk>(raw));
       }
       R = block_max<256>(m, red);
-      sum = weighted = 0.;
+      w.s = w.t = 0.;
       for (int at = p0; at < end; at += STEP) {
         load_part<T, 256, kChunk, 0>(x, tid, at, end, raw);
         fix_part<T, 256, kChunk, 0>(raw, tid, at, end);
         float ps = 0.f, pt = 0.f;
         lane_sums<T, 0, kChunk, ENT, false>(raw, R, 0.f, a.c, ps, pt);
-        sum += ps;
-        if (ENT) weighted += pt;
+        w.s += ps;
+        if (ENT) w.t += pt;
       }
-      s = (float)sum;
-      t = (float)weighted;
+      s = (float)w.s;
+      t = (float)w.t;
       join_waves<256, ENT>(a.c, red, R, s, t);
     }
     if (threadIdx.x == 0) {
@@ -928,7 +971,7 @@ __device__ __forceinline__ float row_kl(const DistillArgs& a, int Kp, Teacher l,
   for (int k = threadIdx.x & 63; k < Kp; k += 64) {
     const float qk = l.q[k];
     if (qk == 0.f) continue;  // NaN is not 0: it reaches the loss
-    const float lp = empty ? -INFINITY : (l.x[k] - R) * a.v.scale - logs;
+    const float lp = empty ? -INFINITY : __builtin_fmaf(l.x[k] - R, a.v.scale, -logs);
     kl += qk * (l.logq[k] - lp);
   }
   return wave64_sum(kl);

@@ -257,7 +257,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
     ``logits`` [..., V] f32 or bf16, ``tokens`` [...] int64 or int32.  ``entropy=True`` adds the entropy of
     each position's distribution (in nats), ``top_k`` (up to 64) its most likely tokens and their log
     probabilities, best first; equal logits are ordered by their id.  Gradients flow to the logits from
-    ``logp`` and ``entropy``, none from the alternatives.
+    ``logp`` and ``entropy``, none from the alternatives.  Sums are f32: both are off by some 1e-6, and by f32's rounding
+    of their own size.
 
     * a negative token marks padding: logp 0, entropy 0, no alternatives, gradient 0, whatever its logits hold;
     * a logit of -inf is a masked token: probability 0, never an alternative.  With fewer than ``top_k``
