@@ -322,6 +322,27 @@ __global__ void __launch_bounds__(1024) ln_cols_kernel(const float* __restrict__
 // (red: a row of 16 floats, all of which are written: 1024 threads are 16 waves)
 __device__ __forceinline__ float block1024_sum(float v, float* red) { return group_sum<0, 1024>(v, red); }
 
+// Sums of term(i, a, b) over i = from, from + step, ... < to: in pieces of 16 terms, which are added up in 64 bits (one after
+// the other in f32 their roundings grow with the number of terms: a thread of a row of 2^24 columns has 16384).  All loads
+// of a piece are in flight at once: 5000 rows of 20000 in bf16, forward, 250 -> 169 us
+template <typename I, typename F>
+__device__ __forceinline__ void long_sums(I from, I to, I step, float& a, float& b, F term) {
+  double sa = 0., sb = 0.;
+  for (; from + 15 * step < to; from += 16 * step) {
+    float pa = 0.f, pb = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) term(from + k * step, pa, pb);
+    sa += pa;
+    sb += pb;
+  }
+  float pa = 0.f, pb = 0.f;
+  for (; from < to; from += step) term(from, pa, pb);
+  sa += pa;
+  sb += pb;
+  a = (float)sa;
+  b = (float)sb;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const LayerNormArgs a) {
   __shared__ __attribute__((aligned(16))) float red[2][16];
@@ -329,13 +350,13 @@ __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const LayerNormArgs a
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     T* y = static_cast<T*>(a.y) + row * a.C;
-    float s = 0.f, q = 0.f;
-    for (int i = threadIdx.x; i < a.C; i += 1024) s += elem_f32(x[i]);
+    float s, q, unused;
+    long_sums((int)threadIdx.x, a.C, 1024, s, unused, [&](int i, float& p, float&) { p += elem_f32(x[i]); });
     const float mean = block1024_sum(s, red[0]) * inv_c;
-    for (int i = threadIdx.x; i < a.C; i += 1024) {
+    long_sums((int)threadIdx.x, a.C, 1024, q, unused, [&](int i, float& p, float&) {
       const float d = elem_f32(x[i]) - mean;
-      q += d * d;
-    }
+      p += d * d;
+    });
     const float r = __builtin_amdgcn_rsqf(block1024_sum(q, red[1]) * inv_c + a.eps);
     for (int i = threadIdx.x; i < a.C; i += 1024)
       elem_st(y + i, (elem_f32(x[i]) - mean) * r * (a.gamma ? a.gamma[i] : 1.f) + (a.beta ? a.beta[i] : 0.f));
@@ -352,12 +373,12 @@ __global__ void __launch_bounds__(1024) ln_bwd_wide_kernel(const LayerNormArgs a
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     T* dx = static_cast<T*>(a.dx) + row * a.C;
     const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
-    float s1 = 0.f, s2 = 0.f;
-    for (int i = threadIdx.x; i < a.C; i += 1024) {
+    float s1, s2;
+    long_sums((int)threadIdx.x, a.C, 1024, s1, s2, [&](int i, float& p1, float& p2) {
       const float g = elem_f32(dy[i]) * (a.gamma ? a.gamma[i] : 1.f);
-      s1 += g;
-      s2 += g * (elem_f32(x[i]) - st.x) * st.y;
-    }
+      p1 += g;
+      p2 += g * (elem_f32(x[i]) - st.x) * st.y;
+    });
     s1 = block1024_sum(s1, red[0]) * inv_c;
     s2 = block1024_sum(s2, red[1]) * inv_c;
     for (int i = threadIdx.x; i < a.C; i += 1024) {
@@ -374,13 +395,13 @@ __global__ void __launch_bounds__(256) ln_cols_wide_kernel(const LayerNormArgs a
   if (c >= a.C) return;
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
-  float dg = 0.f, db = 0.f;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+  float dg, db;
+  long_sums((int64_t)blockIdx.y, a.rows, (int64_t)gridDim.y, dg, db, [&](int64_t row, float& pg, float& pb) {
     const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
     const float d = elem_f32(dy[row * a.dy_stride + c]);
-    dg += d * (elem_f32(x[row * a.stride + c]) - st.x) * st.y;
-    db += d;
-  }
+    pg += d * (elem_f32(x[row * a.stride + c]) - st.x) * st.y;
+    pb += d;
+  });
   float* part = a.part + (int64_t)blockIdx.y * 2 * a.C;
   part[c] = dg;
   part[a.C + c] = db;

@@ -4,7 +4,7 @@ import math
 import lm_oracle as oracle
 import pytest
 import torch
-from test_lm_ops_cpu import check_distill, check_tokens, teacher_rows
+from test_lm_ops_cpu import _norm_vars, check_distill, check_tokens, teacher_rows
 
 from tensorflow_examples_amd import ops
 
@@ -140,3 +140,28 @@ def test_values_far_from_zero_and_from_what_comes_first(gpu, rows, V, dtype):
         y[0, V // 2], y[1, 0], y[2, V - 1], y[3, V // 2] = bad, bad, bad, bad
         r = ops.token_log_probs(y, tok[:4] % V, entropy=True, top_k=3)
         assert torch.isnan(r.logp).all() and torch.isnan(r.entropy).all()
+
+
+def test_layer_norm_of_very_wide_equal_rows(gpu):
+    """The mean of 2^22 equal values: up to 32 terms in f32 at a time (31 roundings), 64 bits, the tree (10), the division (2); what
+    it is off is scaled by 1 / sqrt(eps)"""
+    x = torch.full((3, 1 << 22), 0.1, device=gpu)
+    y = ops.layer_norm(x)
+    assert float(y.abs().max()) <= (31 + 1 + 10 + 2) * U * 0.1 / math.sqrt(1e-5)
+
+
+@pytest.mark.parametrize("C", [16400, 600])
+def test_layer_norm_weights_gradients_of_many_equal_rows(gpu, C):
+    """40000 equal rows: blocks or threads of at most 157 rows one after the other, of wide rows up to 32, and 64 bits"""
+    torch.manual_seed(0)
+    rows = 40000
+    _, g, b = _norm_vars(C, gpu)
+    x, dy = torch.randn(1, C, device=gpu), 0.1 + torch.rand(1, C, device=gpu)
+    ops.layer_norm(x.expand(rows, C), g, b).backward(dy.expand(rows, C))
+    xh = (x.double() - x.double().mean()) * torch.rsqrt(x.double().var(unbiased=False) + 1e-5)
+    n = 31 + 20 if C > 16384 else 157 + 24  # of a thread or a group; the joins
+    want = rows * dy.double()[0]
+    assert bool(((b.grad - want).abs() <= n * U * want).all())
+    want = want * xh[0]
+    # the mean is off by 60 U of itself and its standard deviation's 60 U, xh by as much and 4 U of itself
+    assert bool(((g.grad - want).abs() <= n * U * want.abs() + rows * dy[0] * U * (60 + 64 * xh[0].abs())).all())
