@@ -43,6 +43,11 @@ void first_order(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": its gradient cannot be differentiated again (create_graph=True)");
 }
 
+// ... and the passes write into tensors of their own, in which a forward-mode derivative would end
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, ": forward-mode derivatives are not implemented");
+}
+
 bool is_bf16(const Tensor& t, const char* what) {
   const bool b = t.scalar_type() == at::kBFloat16;
   TORCH_CHECK_TYPE(b || t.scalar_type() == at::kFloat, what, ": float32 or bfloat16 expected, got ", t.scalar_type());
@@ -239,6 +244,7 @@ struct TokenLogProbsFn : torch::autograd::Function<TokenLogProbsFn> {
 // (logp [...], entropy [...]?, top_logp [..., K]?, top_ids [..., K]?)
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t top_k,
                                                            bool entropy, double temperature) {
+  no_tangent(logits, "token_log_probs");
   check_matrix(logits, tfx::kVocabMax, "logits");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
   check_side(tokens, logits, lead, -1, "tokens");
@@ -368,6 +374,7 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
 
 Tensor distillation_loss(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double temperature,
                          const optional<Tensor>& weight, bool fuse) {
+  no_tangent(logits, "distillation_loss");
   check_matrix(logits, tfx::kVocabMax, "logits");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
   TORCH_CHECK_VALUE(ids.dim() == logits.dim() && ids.size(-1) >= 1 && ids.size(-1) <= tfx::kDistillMaxTop,
@@ -501,6 +508,7 @@ Tensor layer_norm(const Tensor& input, const optional<Tensor>& anchor, const opt
                   const optional<Tensor>& beta, int64_t beta_at, const optional<Tensor>& dgamma,
                   const optional<Tensor>& dbeta, double eps) {
   TORCH_CHECK_VALUE(eps >= 1e-30 && std::isfinite(eps), "layer_norm: eps of at least 1e-30 expected, got ", eps);
+  no_tangent(input, "layer_norm");
   if (at::GradMode::is_enabled() && (input.requires_grad() || has(anchor)))
     return LayerNormFn::apply(input, anchor, gamma, gamma_at, beta, beta_at, dgamma, dbeta, eps);
   const Tensor x = rows_of(input, tfx::kLayerNormMax, "layer_norm");

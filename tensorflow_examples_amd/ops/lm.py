@@ -10,7 +10,8 @@ ones (any row stride); only elements of a row that are not next to each other co
 ``distillation_loss``   T^2 KL(teacher || student) from the teacher's top logits; differentiable in the
                         student's logits
 
-Gradients are of first order: create_graph=True is refused (on the CPU, what differentiates them again).
+Gradients are of first order and in reverse mode: create_graph=True is refused (on the CPU, what differentiates
+them again), and so is a tensor that carries a forward-mode tangent.
 
 The lists of top alternatives that ``token_log_probs`` returns (id -1 where nothing is left) are the
 teacher's lists that ``distillation_loss`` takes.
