@@ -6,6 +6,7 @@
 // interpreter lock in the engine's thread.  A training step of 6400 rows of 65 logits, bound by the host,
 // takes 57 us with them and took 83 us with nodes in Python.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -14,7 +15,10 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <memory>
+#include <mutex>
 #include <tuple>
+#include <unordered_map>
 
 #include "tfx_kernels.h"
 
@@ -405,6 +409,67 @@ tfx::LayerNormArgs norm_args(const Tensor& x, const float* gamma) {
   return a;
 }
 
+// What a backward pass asks of a variable store when it runs: its gradients' buffer then, and whether it wants to hear of
+// each gradient that is there (variables.py tells; the store's number is its key).
+struct Store {
+  int64_t number = 0;
+  Tensor grad;
+  bool hooked = false;
+};
+std::mutex stores_lock;
+std::unordered_map<int64_t, std::shared_ptr<Store>>& stores() {
+  static std::unordered_map<int64_t, std::shared_ptr<Store>> s;
+  return s;
+}
+
+std::shared_ptr<Store> store_of(int64_t number) {  // below 0: none
+  if (number < 0) return nullptr;
+  const std::lock_guard<std::mutex> l(stores_lock);
+  const auto it = stores().find(number);
+  TORCH_CHECK(it != stores().end(), "no variable store of number ", number);
+  return it->second;
+}
+
+int64_t store_new() {
+  static int64_t next = 0;
+  const std::lock_guard<std::mutex> l(stores_lock);
+  auto s = std::make_shared<Store>();
+  s->number = next;
+  stores()[next] = std::move(s);
+  return next++;
+}
+
+void store_set(int64_t number, const optional<Tensor>& grad, bool hooked) {
+  const auto s = store_of(number);
+  const std::lock_guard<std::mutex> l(stores_lock);
+  s->grad = has(grad) ? *grad : Tensor();
+  s->hooked = hooked;
+}
+
+void store_free(int64_t number) {
+  const std::lock_guard<std::mutex> l(stores_lock);
+  stores().erase(number);
+}
+
+optional<Tensor> grad_of(const std::shared_ptr<Store>& s) {
+  if (!s) return c10::nullopt;
+  const std::lock_guard<std::mutex> l(stores_lock);
+  TORCH_CHECK(s->grad.defined(), "layer_norm: the variable store has no gradients");
+  return s->grad;
+}
+
+// The store's hook, in Python (ops/lm.py), for the variable at element `at`
+void tell_ready(const std::shared_ptr<Store>& s, int64_t at) {
+  if (!s) return;
+  {
+    const std::lock_guard<std::mutex> l(stores_lock);
+    if (!s->hooked) return;
+  }
+  static const auto ready =
+      c10::Dispatcher::singleton().findSchemaOrThrow("tfx::grad_ready", "").typed<void(int64_t, int64_t)>();
+  ready.call(s->number, at);
+}
+
 // C elements of a variable store's flat f32 buffer
 float* var_or_null(const optional<Tensor>& flat, int64_t offset, const Tensor& x, const char* what) {
   if (!has(flat)) return nullptr;
@@ -465,17 +530,18 @@ Tensor norm_pass_bwd(const Tensor& x, const Tensor& gy, const Tensor& stats, con
 }
 
 struct NormKept : torch::CustomClassHolder {
-  optional<Tensor> gamma, dgamma, dbeta;  // flat buffers
+  optional<Tensor> gamma;                   // flat buffer
+  std::shared_ptr<Store> gammas, betas;     // whose gradients are wanted
   int64_t gamma_at = 0, beta_at = 0;
   bool want_dx = false;
 };
 
 // The weights are slices of their stores' flat buffers (variables.py), whose gradients the backward pass adds
-// to; `anchor` is the leaf that records a call whose input needs no gradient.
+// to (those of gamma_store and beta_store; below 0: not wanted); `anchor` is the leaf that records a call whose input needs no gradient.
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& input, const optional<Tensor>& anchor,
                         const optional<Tensor>& gamma, int64_t gamma_at, const optional<Tensor>& beta, int64_t beta_at,
-                        const optional<Tensor>& dgamma, const optional<Tensor>& dbeta, double eps) {
+                        int64_t gamma_store, int64_t beta_store, double eps) {
     const Tensor x = rows_of(input, tfx::kLayerNormMax, "layer_norm");
     auto [y, stats] = norm_pass(x, input.sizes(), var_or_null(gamma, gamma_at, x, "gamma"),
                                 var_or_null(beta, beta_at, x, "beta"), eps, true);
@@ -483,8 +549,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     // (not saved variables: an optimizer may write them before a later backward pass, as with every other op)
     auto k = c10::make_intrusive<NormKept>();
     k->gamma = gamma;
-    k->dgamma = dgamma;
-    k->dbeta = dbeta;
+    k->gammas = store_of(gamma_store);
+    k->betas = store_of(beta_store);
     k->gamma_at = gamma_at;
     k->beta_at = beta_at;
     k->want_dx = input.requires_grad();
@@ -498,19 +564,20 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const Tensor& x = saved[0];
     const auto k = kept<NormKept>(ctx);
     out[0] = norm_pass_bwd(x, g[0], saved[1], var_or_null(k->gamma, k->gamma_at, x, "gamma"),
-                           var_or_null(k->dgamma, k->gamma_at, x, "gamma"), var_or_null(k->dbeta, k->beta_at, x, "beta"),
-                           k->want_dx);
+                           var_or_null(grad_of(k->gammas), k->gamma_at, x, "gamma"),
+                           var_or_null(grad_of(k->betas), k->beta_at, x, "beta"), k->want_dx);
+    tell_ready(k->gammas, k->gamma_at);
+    tell_ready(k->betas, k->beta_at);
     return out;
   }
 };
 
 Tensor layer_norm(const Tensor& input, const optional<Tensor>& anchor, const optional<Tensor>& gamma, int64_t gamma_at,
-                  const optional<Tensor>& beta, int64_t beta_at, const optional<Tensor>& dgamma,
-                  const optional<Tensor>& dbeta, double eps) {
+                  const optional<Tensor>& beta, int64_t beta_at, int64_t gamma_store, int64_t beta_store, double eps) {
   TORCH_CHECK_VALUE(eps >= 1e-30 && std::isfinite(eps), "layer_norm: eps of at least 1e-30 expected, got ", eps);
   no_tangent(input, "layer_norm");
   if (at::GradMode::is_enabled() && (input.requires_grad() || has(anchor)))
-    return LayerNormFn::apply(input, anchor, gamma, gamma_at, beta, beta_at, dgamma, dbeta, eps);
+    return LayerNormFn::apply(input, anchor, gamma, gamma_at, beta, beta_at, gamma_store, beta_store, eps);
   const Tensor x = rows_of(input, tfx::kLayerNormMax, "layer_norm");
   return std::get<0>(norm_pass(x, input.sizes(), var_or_null(gamma, gamma_at, x, "gamma"),
                                var_or_null(beta, beta_at, x, "beta"), eps, false));
@@ -538,8 +605,11 @@ Tensor layer_norm_bwd(const Tensor& input, const Tensor& dy, const Tensor& stats
 TORCH_LIBRARY_FRAGMENT(tfx, m) {
   m.def("token_log_probs", &token_log_probs);
   m.def("distillation_loss", &distillation_loss);
-  m.def("layer_norm(Tensor x, Tensor? anchor, Tensor? gamma, int gamma_at, Tensor? beta, int beta_at, Tensor(a!)? dgamma, "
-        "Tensor(b!)? dbeta, float eps) -> Tensor", &layer_norm);
+  m.def("layer_norm(Tensor x, Tensor? anchor, Tensor? gamma, int gamma_at, Tensor? beta, int beta_at, int gamma_store, "
+        "int beta_store, float eps) -> Tensor", &layer_norm);
+  m.def("store_new", &store_new);
+  m.def("store_set", &store_set);
+  m.def("store_free", &store_free);
   m.def("layer_norm_fwd", &layer_norm_fwd);
   m.def("layer_norm_bwd(Tensor x, Tensor dy, Tensor stats, Tensor? gamma, Tensor(a!)? dgamma, Tensor(b!)? dbeta, "
         "bool want_dx) -> Tensor", &layer_norm_bwd);

@@ -19,6 +19,7 @@ teacher's lists that ``distillation_loss`` takes.
 from __future__ import annotations
 
 import math
+import weakref
 from typing import NamedTuple, Optional
 
 import torch
@@ -92,6 +93,45 @@ def _ln_bwd_ref(x, dy, stats, gamma, dgamma, dbeta, want_dx):
     return dx.to(x.dtype)
 
 
+class _Watcher:
+    """Keeps the GPU's nodes informed of a store: where its gradients are, and whether it has a hook, as of the
+    backward pass (csrc/torch_ops/lm_ops.cpp).  A copy of the store gets one of its own."""
+    stores: "weakref.WeakValueDictionary[int, object]" = weakref.WeakValueDictionary()
+
+    def __init__(self, store):
+        self.number = torch.ops.tfx.store_new()
+        weakref.finalize(self, torch.ops.tfx.store_free, self.number).atexit = False
+        _Watcher.stores[self.number] = store
+        self.update(store)
+
+    def update(self, store) -> None:
+        torch.ops.tfx.store_set(self.number, store.grad, store.grad_ready_hook is not None)
+
+    def __deepcopy__(self, memo):
+        return None
+
+    def __reduce__(self):
+        return type(None), ()
+
+
+def _store_number(store) -> int:
+    if store.watcher is None:
+        store.watcher = _Watcher(store)
+    return store.watcher.number
+
+
+def _ready(number: int, at: int) -> None:
+    """The variable at element ``at`` of that store has its gradient (called by the GPU's nodes)."""
+    store = _Watcher.stores.get(number)
+    if store is not None:
+        _grad_ready(next(v for v in store.vars if v.offset == at and v.numel))
+
+
+_library = torch.library.Library("tfx", "FRAGMENT")
+_library.define("grad_ready(int store, int at) -> ()")
+_library.impl("grad_ready", _ready, "CompositeExplicitAutograd")
+
+
 class _LayerNorm(torch.autograd.Function):
     """The CPU's node, and the GPU's where a gradient hook has to run after the backward pass."""
 
@@ -153,7 +193,7 @@ def layer_norm(x: torch.Tensor, gamma: Optional[Variable] = None, beta: Optional
         gs, bs = gamma and gamma.store, beta and beta.store
         return torch.ops.tfx.layer_norm(
             x, anchor, gs and gs.master, gamma.offset if gs else 0, bs and bs.master, beta.offset if bs else 0,
-            gs.grad if gs and gamma.trainable else None, bs.grad if bs and beta.trainable else None, eps)
+            _store_number(gs) if gs and gamma.trainable else -1, _store_number(bs) if bs and beta.trainable else -1, eps)
     _check_matrix(x, "layer_norm")
     if not (eps >= 1e-30 and math.isfinite(eps)):
         raise ValueError("layer_norm: eps of at least 1e-30 expected, got %r" % eps)

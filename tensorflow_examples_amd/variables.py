@@ -262,6 +262,7 @@ class VariableStore:
         self.sparse: List[SparseVariable] = []
         self.by_name: Dict[str, Variable] = {}
         self.state: Dict[str, torch.Tensor] = {}  # non-trainable state (BN running stats, global_step)
+        self.watcher = None  # told when grad or grad_ready_hook is set (ops/lm.py)
         self.master: Optional[torch.Tensor] = None
         self.grad: Optional[torch.Tensor] = None
         # True while the gradient buffer is known to be all zeros (a fresh buffer, or the optimizer
@@ -283,6 +284,28 @@ class VariableStore:
         self.grad_ready_hook = None
         self._scopes: List[str] = []
         self._name_counts: Dict[str, int] = {}
+
+    @property
+    def grad(self) -> Optional[torch.Tensor]:
+        """The flat gradient buffer (f32)."""
+        return self._grad
+
+    @grad.setter
+    def grad(self, t: Optional[torch.Tensor]) -> None:
+        self._grad = t
+        if self.watcher is not None:
+            self.watcher.update(self)
+
+    @property
+    def grad_ready_hook(self) -> Optional[Callable]:
+        """Called with each variable when a backward pass has written its gradient."""
+        return self._grad_ready_hook
+
+    @grad_ready_hook.setter
+    def grad_ready_hook(self, f: Optional[Callable]) -> None:
+        self._grad_ready_hook = f
+        if self.watcher is not None:
+            self.watcher.update(self)
 
     # -- naming (tf.name_scope + tf.Variable auto-naming "Variable", "Variable_1", ...)
     def scope(self, name: str):
