@@ -462,14 +462,14 @@ template <typename T>
 void fwd_launch(const LayerNormArgs& a, hipStream_t st) {
   const LnShape s = ln_shape<T>(a.C);
   if (!s.nv) {
-    ln_fwd_wide_kernel<T><<<(int)std::min<int64_t>(a.rows, 4096), 1024, 0, st>>>(a);
+    launch(ln_fwd_wide_kernel<T>, (int)std::min<int64_t>(a.rows, 4096), 1024, 0, st, a);
     return;
   }
   // as many waves as are resident at once (6400 rows of 512 in bf16: 1600 blocks 5.4 us, 256 blocks 7.6; 16384 rows of
   // 8192: 1024 blocks 89 us, 6.0 TB/s).  Of more than 8 waves one or two blocks fit a CU: two a CU, or the last ones run
   // alone (in bf16, 14648 rows of 10240: 819 blocks 171 us, 512 143; 10463 of 14336: 585 blocks 146, 512 117)
   const int grid = (int)ln_grid(s, a.rows, s.lanes ? 2048 : s.waves > 8 ? 512 : 8192 / s.waves);
-#define GO(L, NV, MAXT, SH) ln_fwd_kernel<T, L, NV, MAXT, SH><<<grid, ln_threads(s), 0, st>>>(a)
+#define GO(L, NV, MAXT, SH) launch(ln_fwd_kernel<T, L, NV, MAXT, SH>, grid, ln_threads(s), 0, st, a)
   LN_SHAPES(GO);
 #undef GO
 }
@@ -479,14 +479,14 @@ void bwd_launch(const LayerNormArgs& a, hipStream_t st) {
   const LnShape s = ln_shape<T>(a.C);
   const int parts = layer_norm_parts(a.bf16, a.rows, a.C);
   if (!s.nv) {
-    if (a.dx) ln_bwd_wide_kernel<T><<<(int)std::min<int64_t>(a.rows, 4096), 1024, 0, st>>>(a);
-    if (a.part) ln_cols_wide_kernel<T><<<dim3((a.C + 255) / 256, parts), 256, 0, st>>>(a);
+    if (a.dx) launch(ln_bwd_wide_kernel<T>, (int)std::min<int64_t>(a.rows, 4096), 1024, 0, st, a);
+    if (a.part) launch(ln_cols_wide_kernel<T>, dim3((a.C + 255) / 256, parts), 256, 0, st, a);
   } else {
-#define GO(L, NV, MAXT, SH) ln_bwd_kernel<T, L, NV, MAXT, SH><<<parts, ln_threads(s), 0, st>>>(a)
+#define GO(L, NV, MAXT, SH) launch(ln_bwd_kernel<T, L, NV, MAXT, SH>, parts, ln_threads(s), 0, st, a)
     LN_SHAPES(GO);
 #undef GO
   }
-  if (a.part) ln_cols_kernel<<<(2 * a.C + 63) / 64, 1024, 0, st>>>(a.part, parts, a.C, a.dgamma, a.dbeta);
+  if (a.part) launch(ln_cols_kernel, (2 * a.C + 63) / 64, 1024, 0, st, a.part, parts, a.C, a.dgamma, a.dbeta);
 }
 
 }  // namespace

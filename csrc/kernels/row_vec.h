@@ -6,9 +6,28 @@
 // touches.  The last vector of a row is read as the row's last 16 bytes and shifted into place when it is
 // used (vec_ld_near, vec_fix): one load like all others, with no per-element loads and no branch around it.
 #pragma once
+#include <stdexcept>
+#include <tuple>
+
 #include "tfx_common.h"
 
 namespace tfx {
+
+// A launch that says itself whether the runtime took it.  (What hipGetLastError holds behind <<<>>> may be the error of an
+// earlier call of another's, which is its owner's to take.)
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 grid, int threads, size_t lds, hipStream_t s, A... args) {
+  std::tuple<P...> held(args...);
+  const hipError_t e = std::apply(
+      [&](auto&... v) {
+        void* at[] = {const_cast<void*>(static_cast<const void*>(&v))...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), at, lds, s);
+      },
+      held);
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();  // this launch's
+  throw std::runtime_error(hipGetErrorString(e));
+}
 
 template <typename T>
 struct Vec;  // elements of a 16-byte vector

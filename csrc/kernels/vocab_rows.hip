@@ -1250,16 +1250,16 @@ void stats_launch(const VocabArgs& a, Shape s, hipStream_t st) {
   if (s.tpb == 64) {
 #define GO(NV)                                                                                              \
   if (s.nv == NV)                                                                                           \
-    vocab_stats_kernel<T, NV, ENT, TOP><<<grid, 64, TOP ? (size_t)top_room<T, NV>(a.K) * 8 : 0, st>>>(a)
+    launch(vocab_stats_kernel<T, NV, ENT, TOP>, grid, 64, TOP ? (size_t)top_room<T, NV>(a.K) * 8 : 0, st, a)
     GO(1); GO(2); GO(4); GO(8);
     GO(10); GO(12); GO(14); GO(16);
 #undef GO
     return;
   }
-  vocab_stream_kernel<T, ENT, TOP><<<grid, 256, 0, st>>>(a);
+  launch(vocab_stream_kernel<T, ENT, TOP>, grid, 256, 0, st, a);
   if (a.nparts == 1) return;
   const size_t jl = TOP ? ((size_t)a.K * a.K + (size_t)a.nparts * heads_of(a.nparts, a.K)) * 8 : 0;
-  vocab_join_kernel<T, TOP><<<grid_of(a.rows), 256, jl, st>>>(a);
+  launch(vocab_join_kernel<T, TOP>, grid_of(a.rows), 256, jl, st, a);
 }
 
 template <typename T>
@@ -1308,7 +1308,7 @@ template <typename T, int TPB, int NV>
 void fused_go(const DistillArgs& a, T* dx, hipStream_t st) {
   constexpr bool AHEAD = TPB == 1024;
   const int grid = std::min(grid_of(a.v.rows), AHEAD ? 256 : kMaxGrid);
-  distill_fused_kernel<T, TPB, NV, AHEAD><<<grid, TPB, (size_t)((a.K + 3) & ~3) * 16, st>>>(a, dx);
+  launch(distill_fused_kernel<T, TPB, NV, AHEAD>, grid, TPB, (size_t)((a.K + 3) & ~3) * 16, st, a, dx);
 }
 
 template <typename T>
@@ -1332,8 +1332,8 @@ void vocab_bwd_launch(VocabArgs a, const float* g_logp, const float* g_ent, void
   T* d = static_cast<T*>(dx);
 #define GO(TPB, NV)                                                                                       \
   do {                                                                                                    \
-    if (g_ent) vocab_bwd_kernel<T, TPB, NV, true><<<grid, TPB, 0, st>>>(a, g_logp, g_ent, d);             \
-    else vocab_bwd_kernel<T, TPB, NV, false><<<grid, TPB, 0, st>>>(a, g_logp, g_ent, d);                  \
+    if (g_ent) launch(vocab_bwd_kernel<T, TPB, NV, true>, grid, TPB, 0, st, a, g_logp, g_ent, d);             \
+    else launch(vocab_bwd_kernel<T, TPB, NV, false>, grid, TPB, 0, st, a, g_logp, g_ent, d);                  \
   } while (0)
   if (s.tpb == 256) GO(256, 4);
   else if (s.nv == 1) GO(64, 1);
@@ -1349,7 +1349,7 @@ void distill_bwd_launch(DistillArgs a, const float* g, void* dx, hipStream_t st)
   const int grid = grid_of((int64_t)a.v.rows * a.v.nparts);
   const size_t lds = (size_t)((a.K + 3) & ~3) * 16;
   T* d = static_cast<T*>(dx);
-#define GO(TPB, NV) distill_bwd_kernel<T, TPB, NV><<<grid, TPB, lds, st>>>(a, g, d)
+#define GO(TPB, NV) launch(distill_bwd_kernel<T, TPB, NV>, grid, TPB, lds, st, a, g, d)
   if (s.tpb == 256) GO(256, 4);
   else if (s.nv == 1) GO(64, 1);
   else if (s.nv == 2) GO(64, 2);
@@ -1377,15 +1377,15 @@ bool distill_fits(bool bf16, int64_t V) {
 
 void distill_fused(const DistillArgs& a, void* dx, float* loss, hipStream_t st) {
   a.v.bf16 ? fused_launch<uint16_t>(a, dx, st) : fused_launch<float>(a, dx, st);
-  rows_sum_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.v.rows, loss);
+  launch(rows_sum_kernel, 1, 1024, 0, st, a.loss_rows, a.v.rows, loss);
 }
 
 void distill_loss(const DistillArgs& a, float* loss, hipStream_t st) {
   const int grid = grid_of(a.v.rows);
   const size_t lds = (size_t)((a.K + 3) & ~3) * 16;
-  if (a.v.bf16) distill_loss_kernel<uint16_t><<<grid, 64, lds, st>>>(a);
-  else distill_loss_kernel<float><<<grid, 64, lds, st>>>(a);
-  rows_sum_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.v.rows, loss);
+  if (a.v.bf16) launch(distill_loss_kernel<uint16_t>, grid, 64, lds, st, a);
+  else launch(distill_loss_kernel<float>, grid, 64, lds, st, a);
+  launch(rows_sum_kernel, 1, 1024, 0, st, a.loss_rows, a.v.rows, loss);
 }
 
 void distill_bwd(const DistillArgs& a, const float* g, void* dx, hipStream_t st) {
@@ -1396,8 +1396,8 @@ void scale_unless_one(void* x, bool bf16, int64_t n, const float* g, hipStream_t
   // two blocks a CU: mostly they read one number and end, in 2 us
   const int64_t per = (int64_t)1024 * (bf16 ? 8 : 4);
   const int grid = (int)std::min<int64_t>(512, (n + per - 1) / per);
-  if (bf16) scale_unless_one_kernel<uint16_t><<<grid, 1024, 0, st>>>(static_cast<uint16_t*>(x), n, g);
-  else scale_unless_one_kernel<float><<<grid, 1024, 0, st>>>(static_cast<float*>(x), n, g);
+  if (bf16) launch(scale_unless_one_kernel<uint16_t>, grid, 1024, 0, st, static_cast<uint16_t*>(x), n, g);
+  else launch(scale_unless_one_kernel<float>, grid, 1024, 0, st, static_cast<float*>(x), n, g);
 }
 
 }  // namespace tfx

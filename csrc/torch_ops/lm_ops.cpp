@@ -17,6 +17,7 @@
 #include <cmath>
 #include <memory>
 #include <mutex>
+#include <stdexcept>
 #include <tuple>
 #include <unordered_map>
 
@@ -31,16 +32,15 @@ namespace {
 
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
-// A launch that the runtime refuses leaves an error behind, not a result.  What an earlier call of another's left is
-// not taken for it.
-struct Launch {
-  const char* what;
-  explicit Launch(const char* w) : what(w) { (void)hipGetLastError(); }
-  void done() const {
-    const hipError_t e = hipGetLastError();
-    TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+// A launch that the runtime refuses leaves no result
+template <typename F>
+void launching(const char* what, F f) {
+  try {
+    f();
+  } catch (const std::runtime_error& e) {
+    TORCH_CHECK(false, what, ": ", e.what());
   }
-};
+}
 
 // the backward kernels leave no graph of their own: create_graph=True would give gradients without one
 void first_order(const char* what) {
@@ -188,9 +188,9 @@ TokenResult token_pass(const Tensor& x, const Tensor& tokens, at::IntArrayRef le
   }
   if (a.rows) {
     with_parts(a, x, ws, keys);
-    const Launch l("token_log_probs");
-    tfx::vocab_stats(a, stream_of(x));
-    l.done();
+    launching("token_log_probs", [&] {
+      tfx::vocab_stats(a, stream_of(x));
+    });
   }
   return r;
 }
@@ -207,9 +207,9 @@ Tensor token_pass_bwd(const Tensor& x, const Tensor& tokens, const Tensor& stats
   c10::DeviceGuard guard(x.device());
   Tensor dx = at::empty(s.shape, x.options());
   if (a.rows) {
-    const Launch l("token_log_probs backward");
-    tfx::vocab_bwd(a, gp, hp, dx.data_ptr(), stream_of(x));
-    l.done();
+    launching("token_log_probs backward", [&] {
+      tfx::vocab_bwd(a, gp, hp, dx.data_ptr(), stream_of(x));
+    });
   }
   return dx;
 }
@@ -303,9 +303,9 @@ DistillResult distill_pass(const Tensor& x, const Tensor& teacher, const Tensor&
   a.loss_rows = rows.data_ptr<float>();
   if (want_grad && fuse && tfx::distill_fits(a.v.bf16, a.v.V)) {
     r.dx = at::empty({a.v.rows, a.v.V}, x.options());
-    const Launch l("distillation_loss");
-    tfx::distill_fused(a, r.dx.data_ptr(), r.loss.data_ptr<float>(), s);
-    l.done();
+    launching("distillation_loss", [&] {
+      tfx::distill_fused(a, r.dx.data_ptr(), r.loss.data_ptr<float>(), s);
+    });
     return r;
   }
   r.stats = at::empty({a.v.rows, 4}, f32);
@@ -317,10 +317,10 @@ DistillResult distill_pass(const Tensor& x, const Tensor& teacher, const Tensor&
     a.coef = r.coef.data_ptr<float>();
   }
   with_parts(a.v, x, ws, keys);
-  const Launch l("distillation_loss");
-  tfx::vocab_stats(a.v, s);
-  tfx::distill_loss(a, r.loss.data_ptr<float>(), s);
-  l.done();
+  launching("distillation_loss", [&] {
+    tfx::vocab_stats(a.v, s);
+    tfx::distill_loss(a, r.loss.data_ptr<float>(), s);
+  });
   return r;
 }
 
@@ -351,9 +351,9 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
       const float* s = f32_or_null(seed, dx, 1, "the loss's gradient");
       if (dx.numel()) {
         c10::DeviceGuard guard(dx.device());
-        const Launch l("distillation_loss backward");
-        tfx::scale_unless_one(dx.data_ptr(), is_bf16(dx, "dx"), dx.numel(), s, stream_of(dx));
-        l.done();
+        launching("distillation_loss backward", [&] {
+          tfx::scale_unless_one(dx.data_ptr(), is_bf16(dx, "dx"), dx.numel(), s, stream_of(dx));
+        });
       }
       out[0] = k->shape.size() == 2 ? std::move(dx) : dx.view(k->shape);
       return out;
@@ -368,9 +368,9 @@ struct DistillationFn : torch::autograd::Function<DistillationFn> {
     c10::DeviceGuard guard(x.device());
     out[0] = at::empty(k->shape, x.options());
     if (a.v.rows) {
-      const Launch l("distillation_loss backward");
-      tfx::distill_bwd(a, s, out[0].data_ptr(), stream_of(x));
-      l.done();
+      launching("distillation_loss backward", [&] {
+        tfx::distill_bwd(a, s, out[0].data_ptr(), stream_of(x));
+      });
     }
     return out;
   }
@@ -493,9 +493,9 @@ std::tuple<Tensor, Tensor> norm_pass(const Tensor& x, at::IntArrayRef shape, con
     a.stats = st.data_ptr<float>();
   }
   if (a.rows) {
-    const Launch l("layer_norm");
-    tfx::layer_norm_fwd(a, stream_of(x));
-    l.done();
+    launching("layer_norm", [&] {
+      tfx::layer_norm_fwd(a, stream_of(x));
+    });
   }
   return {y, st};
 }
@@ -523,9 +523,9 @@ Tensor norm_pass_bwd(const Tensor& x, const Tensor& gy, const Tensor& stats, con
     part = at::empty({tfx::layer_norm_parts(a.bf16, a.rows, a.C), 2, a.C}, x.options().dtype(at::kFloat));
     a.part = part.data_ptr<float>();
   }
-  const Launch l("layer_norm backward");
-  tfx::layer_norm_bwd(a, stream_of(x));
-  l.done();
+  launching("layer_norm backward", [&] {
+    tfx::layer_norm_bwd(a, stream_of(x));
+  });
   return dx;
 }
 

@@ -1,5 +1,6 @@
 """Calls of layer norm, token log probabilities and distillation that their programs make rarely."""
 import copy
+import ctypes
 import gc
 import pickle
 
@@ -96,3 +97,27 @@ def test_layer_norm_of_copied_and_of_gone_stores(gpu):
     gc.collect()
     y.backward(dy)  # the node keeps what it writes to
     assert torch.isfinite(leaf.grad).all()
+
+
+def test_an_earlier_error_of_anothers_stays_its_owners(gpu):
+    """A refused runtime call (a device that is not there) leaves an error on this thread: the operators neither take it for
+    theirs nor take it away"""
+    path = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+    hip = ctypes.CDLL(path)
+    x = torch.randn(6, 300, device=gpu)
+    tok = torch.zeros(6, dtype=torch.long, device=gpu)
+    t, ids = teacher_rows(6, 300, 3, gpu)
+    torch.cuda.synchronize()
+    hip.hipGetLastError()
+    assert hip.hipSetDevice(1000) != 0
+    left = hip.hipPeekAtLastError()
+    try:
+        if left == 0:
+            pytest.skip("this runtime keeps no error of a refused call")
+        with torch.no_grad():
+            ops.token_log_probs(x, tok, top_k=2, entropy=True)
+            ops.distillation_loss(x, t, ids)
+            ops.layer_norm(x)
+        assert hip.hipPeekAtLastError() == left
+    finally:
+        hip.hipGetLastError()
