@@ -8,7 +8,6 @@ step is captured once into a HIP graph and replayed (launch-bound small models).
 """
 from __future__ import annotations
 
-import time
 from typing import Callable, Optional
 
 import torch
@@ -20,6 +19,17 @@ from .optim import Optimizer
 from .parallel.allreduce import GradAllReduce
 from .utils import trace
 from .variables import VariableStore
+
+
+def retire_collectives(group=None) -> None:
+    """Wait until the watchdogs of ``group`` (None: the default one) and of the default group hold none of the collectives
+    issued so far.  A watchdog asks for their events until it has seen them done, and HIP refuses that for an event of a
+    stream that is capturing meanwhile -- which ends the process: called in front of a capture."""
+    torch.cuda.synchronize()  # done on the device; the watchdogs see it when they look the next time
+    world = dist.group.WORLD
+    for g in [world] + ([group] if group is not None and group is not world else []):
+        if dist.get_backend(g) == "nccl":
+            g._wait_for_pending_works()
 
 
 class ClassifierTrainer:
@@ -109,12 +119,8 @@ class ClassifierTrainer:
                 for _ in range(warmup):
                     self._step(sx, sy)
             torch.cuda.current_stream().wait_stream(s)
-            if self.dp is not None and dist.is_initialized() and dist.get_backend() == "nccl":
-                # The watchdog asks for the warm-up collectives' events until it has seen them done, and HIP
-                # refuses that for an event of a stream that is capturing meanwhile -- which ends the process.
-                # It looks every 100 ms: let it retire them all before their stream is captured.
-                torch.cuda.synchronize()
-                time.sleep(0.5)
+            if self.dp is not None and dist.is_initialized():
+                retire_collectives(getattr(self.dp, "group", None))
             g = torch.cuda.CUDAGraph()
             mode = "thread_local" if self.dp is not None else "global"
             with torch.cuda.graph(g, capture_error_mode=mode):
