@@ -210,29 +210,32 @@ class TokenLogProbs(NamedTuple):
     top_ids: Optional[torch.Tensor]
 
 
-def _lse_ref(z):
-    """Row-wise log sum exp [rows, 1]; -inf for a row of -inf."""
-    m = z.amax(1, keepdim=True)
-    m = torch.where(m == -math.inf, torch.zeros_like(m), m)
-    return m + torch.log(torch.exp(z - m).sum(1, keepdim=True))
+def _log_softmax_ref(x, temperature):
+    """(z, logs, empty) of rows: z = (x - their maximum) / T, log p = z - logs; ``empty`` where nothing but -inf is left (logs
+    is 0 there).  The maximum is taken off first: of a row of the type's lowest value, or far from 0, z would round away."""
+    x = x.float()
+    m = x.amax(1, keepdim=True)
+    z = (x - torch.where(m == -math.inf, torch.zeros_like(m), m)) / temperature
+    s = torch.exp(z).sum(1, keepdim=True)
+    empty = s == 0
+    return z, torch.log(torch.where(empty, torch.ones_like(s), s)), empty
 
 
 def _dist_ref(x, temperature):
-    """(z, lse, p, log p with 0 where p is 0), p = 0 in rows of -inf"""
-    z = x.float() / temperature
-    lse = _lse_ref(z)
-    logq = z - torch.where(lse == -math.inf, torch.zeros_like(lse), lse)
-    p = torch.exp(logq)
-    return z, lse, p, torch.where(p == 0, torch.zeros_like(p), logq)
+    """(empty, p, log p with 0 where p is 0)"""
+    z, logs, empty = _log_softmax_ref(x, temperature)
+    p = torch.exp(z - logs)
+    return empty, p, torch.where(p == 0, torch.zeros_like(p), z - logs)
 
 
 def _tokens_ref(x, tokens, top_k, temperature):
-    z, lse, p, logq = _dist_ref(x, temperature)
+    z, logs, empty = _log_softmax_ref(x, temperature)
+    _, p, logq = _dist_ref(x, temperature)
     V = x.shape[1]
     t = tokens.long()[:, None]
     real = t >= 0
-    logp = z.gather(1, t.clamp(0, V - 1)) - lse
-    logp = torch.where(lse == -math.inf, lse, logp)
+    logp = z.gather(1, t.clamp(0, V - 1)) - logs
+    logp = torch.where(empty, torch.full_like(logp, -math.inf), logp)
     logp = torch.where(t >= V, torch.full_like(logp, math.nan), logp)
     zero = torch.zeros_like(logp)
     ent = -(p * logq).sum(1, keepdim=True)
@@ -244,7 +247,7 @@ def _tokens_ref(x, tokens, top_k, temperature):
         # stable: equal values in the order of their ids
         order = torch.sort(v, dim=1, descending=True, stable=True)[1][:, :top_k]
         there = some.gather(1, order)
-        top = torch.where(there, z.gather(1, order) - lse, torch.full_like(zero, -math.inf))
+        top = torch.where(there, z.gather(1, order) - logs, torch.full_like(zero, -math.inf))
         ids = torch.where(there, order, torch.full_like(order, -1))
         if ids.shape[1] < top_k:
             pad = (0, top_k - ids.shape[1])
@@ -254,12 +257,12 @@ def _tokens_ref(x, tokens, top_k, temperature):
 
 
 def _tokens_bwd_ref(x, tokens, g, h, temperature):
-    _, lse, p, logq = _dist_ref(x, temperature)
+    empty, p, logq = _dist_ref(x, temperature)
     t = tokens.long()[:, None]
     dz = torch.zeros_like(p)
     if g is not None:
         dz = -p * g[:, None]
-        left = torch.where((lse == -math.inf) | (t < 0) | (t >= x.shape[1]), torch.zeros_like(lse), g[:, None])
+        left = torch.where(empty | (t < 0) | (t >= x.shape[1]), torch.zeros_like(g[:, None]), g[:, None])
         dz.scatter_add_(1, t.clamp(0, x.shape[1] - 1), left)
     if h is not None:
         ent = -(p * logq).sum(1, keepdim=True)
@@ -325,22 +328,20 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, 
 def _teacher_ref(x, teacher, ids, weight, temperature):
     """(teacher's q, log q, rows that learn, rows with an id outside the vocabulary, per-row factor)"""
     there = ids >= 0
-    t = torch.where(there, teacher.float() / temperature, torch.full_like(teacher.float(), -math.inf))
-    lse = _lse_ref(t)
+    t, logs, empty = _log_softmax_ref(torch.where(there, teacher.float(), torch.full_like(teacher.float(), -math.inf)),
+                                      temperature)
     bad = (ids >= x.shape[1]).any(1, keepdim=True)
-    w = weight[:, None] if weight is not None else torch.full_like(lse, 1.0 / max(1, x.shape[0]))
+    w = weight[:, None] if weight is not None else torch.full_like(logs, 1.0 / max(1, x.shape[0]))
     bad = bad & (w != 0)
-    real = there.any(1, keepdim=True) & (lse != -math.inf) & (w != 0) & ~bad
-    logq = t - torch.where(lse == -math.inf, torch.zeros_like(lse), lse)
-    return torch.exp(logq), logq, real, bad, w
+    real = there.any(1, keepdim=True) & ~empty & (w != 0) & ~bad
+    return torch.exp(t - logs), t - logs, real, bad, w
 
 
 def _distill_ref(x, teacher, ids, weight, temperature):
     q, logq, real, bad, w = _teacher_ref(x, teacher, ids, weight, temperature)
-    z = x.float() / temperature
-    lse = _lse_ref(z)
-    at = ids.long().clamp(0, x.shape[1] - 1)
-    logp = torch.where(lse == -math.inf, lse, z.gather(1, at) - lse)
+    z, logs, empty = _log_softmax_ref(x, temperature)
+    logp = z.gather(1, ids.long().clamp(0, x.shape[1] - 1)) - logs
+    logp = torch.where(empty, torch.full_like(logp, -math.inf), logp)
     kl = torch.where((q == 0) | ~real, torch.zeros_like(q), q * (logq - logp)).sum(1, keepdim=True)
     rows = torch.where(real, temperature * temperature * w * kl, torch.zeros_like(kl))
     rows = torch.where(bad, torch.full_like(kl, math.nan), rows)
@@ -349,9 +350,9 @@ def _distill_ref(x, teacher, ids, weight, temperature):
 
 def _distill_bwd_ref(x, teacher, ids, weight, g, temperature):
     q, _, real, bad, w = _teacher_ref(x, teacher, ids, weight, temperature)
-    _, lse, p, _ = _dist_ref(x, temperature)
+    empty, p, _ = _dist_ref(x, temperature)
     dz = p.scatter_add(1, ids.long().clamp(0, x.shape[1] - 1), torch.where(ids >= 0, -q, torch.zeros_like(q)))
-    dz = torch.where(real & (lse != -math.inf), dz * (g * w * temperature), torch.zeros_like(dz))
+    dz = torch.where(real & ~empty, dz * (g * w * temperature), torch.zeros_like(dz))
     return torch.where(bad, torch.full_like(dz, math.nan), dz).to(x.dtype)
 
 
