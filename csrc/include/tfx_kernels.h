@@ -344,10 +344,10 @@ void cast_f32_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s);
 void affine_fwd(const float* x, const float* w, const float* b, int64_t n, int C, float* y, hipStream_t s);
 void affine_bwd(const float* g, const float* x, const float* w, int64_t n, int C, float* dx, float* dw, float* db,
                 hipStream_t s);
-// loss[0] = sum (p - y)^2 ; dp = 2 (p - y) * g[0]
 // n 32-bit words = 0, by a kernel: a memset recorded into a captured graph is a node of its own kind, and such
 // nodes have left wrong values on replays after the first
 void clear_words(void* p, int64_t n, hipStream_t s);
+// loss[0] = sum (p - y)^2 ; dp = 2 (p - y) * g[0]
 void sse_fwd(const float* p, const float* y, int64_t n, float* loss, hipStream_t s);
 void sse_bwd(const float* p, const float* y, const float* g, int64_t n, float* dp, hipStream_t s);
 // dz = g * act'(y) (act 0 none, 1 relu, 2 sigmoid, y = the activation OUTPUT); dbias += column sums

@@ -1223,10 +1223,10 @@ struct Shape {
 };
 
 // Rows that one wave's registers hold take one wave each: up to 16 vectors a lane (16384 rows in bf16 of 3000: 22 us,
-// streamed by blocks 41; of 5000: 32 and 48; of 8000: 50 and 53; 256 rows of 5000: 3.7 and, in parts, 7.1).  With top
+// streamed by blocks 41; of 5000: 31 and 48; of 8000: 49 and 53; 256 rows of 5000: 5.1 and, in parts, 7.1).  With top
 // alternatives a wave is on its own for longer, which takes rows enough to hide it: for up to kFewTop of them 16384 rows
-// in bf16 of 8000, top 5: 63 us, streamed 87; 256 rows of 4096: 7.0 and 6.5; for more of them 16384 rows of 6000, top 20:
-// 79 and 96, of 8000 107 and 97; 2000 rows of 5000 17.1 and 16.9; 256 rows of 3000 9.7 and 7.0.
+// in bf16 of 8000, top 5: 69 us, streamed 87; 256 rows of 4096: 8.0 and 6.5; for more of them 16384 rows of 6000, top 20:
+// 85 and 96, of 8000 107 and 100; 2000 rows of 5000 17.1 and 16.9; 256 rows of 3000 9.7 and 7.7.
 // Longer rows take a block, in parts where the list of their alternatives asks for it (kTopVecs) or rows are so few that
 // there would be less than kFewParts blocks.
 constexpr int kFewParts = 512;
