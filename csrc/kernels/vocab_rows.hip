@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(64) vocab_stats_kernel(const VocabArgs a) {
 
 // Longer rows are streamed, nothing of them stays: a block goes over its part in pieces of kChunk vectors a thread,
 // the next piece's loads ahead of the present one's sums.  The whole row is one part unless rows are few.  (4096 rows
-// of 50000 in bf16: 67 us, 6.1 TB/s; with parts held in registers 105 us and 9 to join them.)
+// of 50000 in bf16: 72 us, 5.7 TB/s; with parts held in registers 105 us and 9 to join them.)
 //
 // Top alternatives ride along: each vector's maximum is compared with a threshold, a lower bound of the K-th largest
 // value (the K-th largest of the lanes' own maxima so far), and where it reaches that, the vector's number is noted.

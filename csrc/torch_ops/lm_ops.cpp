@@ -441,14 +441,19 @@ int64_t store_new() {
 
 void store_set(int64_t number, const optional<Tensor>& grad, bool hooked) {
   const auto s = store_of(number);
+  Tensor g = has(grad) ? *grad : Tensor();  // the former one goes behind the lock
   const std::lock_guard<std::mutex> l(stores_lock);
-  s->grad = has(grad) ? *grad : Tensor();
+  std::swap(s->grad, g);
   s->hooked = hooked;
 }
 
 void store_free(int64_t number) {
+  std::shared_ptr<Store> s;
   const std::lock_guard<std::mutex> l(stores_lock);
-  stores().erase(number);
+  const auto it = stores().find(number);
+  if (it == stores().end()) return;
+  s = std::move(it->second);
+  stores().erase(it);
 }
 
 optional<Tensor> grad_of(const std::shared_ptr<Store>& s) {
