@@ -221,16 +221,15 @@ def _log_softmax_ref(x, temperature):
     return z, torch.log(torch.where(empty, torch.ones_like(s), s)), empty
 
 
-def _dist_ref(x, temperature):
-    """(empty, p, log p with 0 where p is 0)"""
-    z, logs, empty = _log_softmax_ref(x, temperature)
+def _dist_ref(z, logs):
+    """(p, log p with 0 where p is 0)"""
     p = torch.exp(z - logs)
-    return empty, p, torch.where(p == 0, torch.zeros_like(p), z - logs)
+    return p, torch.where(p == 0, torch.zeros_like(p), z - logs)
 
 
 def _tokens_ref(x, tokens, top_k, temperature):
     z, logs, empty = _log_softmax_ref(x, temperature)
-    _, p, logq = _dist_ref(x, temperature)
+    p, logq = _dist_ref(z, logs)
     V = x.shape[1]
     t = tokens.long()[:, None]
     real = t >= 0
@@ -257,7 +256,8 @@ def _tokens_ref(x, tokens, top_k, temperature):
 
 
 def _tokens_bwd_ref(x, tokens, g, h, temperature):
-    empty, p, logq = _dist_ref(x, temperature)
+    z, logs, empty = _log_softmax_ref(x, temperature)
+    p, logq = _dist_ref(z, logs)
     t = tokens.long()[:, None]
     dz = torch.zeros_like(p)
     if g is not None:
@@ -350,8 +350,8 @@ def _distill_ref(x, teacher, ids, weight, temperature):
 
 def _distill_bwd_ref(x, teacher, ids, weight, g, temperature):
     q, _, real, bad, w = _teacher_ref(x, teacher, ids, weight, temperature)
-    empty, p, _ = _dist_ref(x, temperature)
-    dz = p.scatter_add(1, ids.long().clamp(0, x.shape[1] - 1), torch.where(ids >= 0, -q, torch.zeros_like(q)))
+    z, logs, empty = _log_softmax_ref(x, temperature)
+    dz = torch.exp(z - logs).scatter_add(1, ids.long().clamp(0, x.shape[1] - 1), torch.where(ids >= 0, -q, torch.zeros_like(q)))
     dz = torch.where(real & ~empty, dz * (g * w * temperature), torch.zeros_like(dz))
     return torch.where(bad, torch.full_like(dz, math.nan), dz).to(x.dtype)
 
